@@ -519,9 +519,10 @@ MCCLX_API int mcclx_dropout(mcclx_ctx* ctx, void* stream, int dtype, uint64_t ro
  * `ignore_index`, whose loss is 0; the mean is over those that are not (NaN where
  * none is left).  A target outside 0 .. vocab - 1 makes its loss and what its gradient
  * reaches NaN.  `grad` is the gradient of the loss: one float, or one a token for
- * MCCLX_LOSS_NONE.  fp32 matrices are
- * multiplied with fp32's precision; dz, in between the products of a backward pass, is
- * held in 16 bits for 16-bit matrices. */
+ * MCCLX_LOSS_NONE.  fp32 matrices, and dz in between the products of a backward
+ * pass, are multiplied with fp32's precision, whatever the sizes of other rows, for
+ * values down to 2^-100 of the largest finite one of their matrix (dz: of 1).  For
+ * 16-bit matrices dz is rounded to their type, f16 after a factor of 2^14. */
 enum { MCCLX_LOSS_NONE = 0, MCCLX_LOSS_MEAN = 1, MCCLX_LOSS_SUM = 2 };
 typedef struct {
     int32_t dtype;     /* of hidden, weight and their gradients */

@@ -8,9 +8,13 @@
 // writes dz of the piece in 16 bits; then the piece's rows of dw, which no other piece touches, and its share
 // of dh, which adds up in fp32.  8 tokens x vocab x width flops in all, on the matrix cores.
 //
-// fp32 operands are split into two f16 planes, x s = hi + 2^-11 lo with s a power of two that brings the tensor's
-// largest value to 2^14: 22 bits and the sign, and three products lo hi + hi lo, then hi hi, in place of one; the term lo lo is
-// below fp32's own rounding.  (The matrix cores multiply fp32 at a sixteenth of f16's rate.)
+// fp32 operands, dz among them, are split into three bf16 planes, x = x0 + x1 + x2 exactly, 8 bits each, and six products of planes, x1 y1,
+// x0 y2, x2 y0, x0 y1, x1 y0, x0 y0, take the place of one: what is left out is below 2^-25 of a product, half of an fp32 rounding.  (The
+// matrix cores multiply fp32 at a sixteenth of bf16's rate.)  bf16 has fp32's exponents, so that a large row costs the others
+// nothing; all that has to be seen to is that products neither overflow nor vanish, and a power of two that brings a matrix's largest
+// value to 2^50 does that for values down to 2^-100 of it (fp32 itself cannot multiply all that it holds).  Two f16 planes and three
+// products would take 0.6 of the time (4096 tokens, 32000 x 768, forward and backward 2.4 ms, this way 4.1), but hold 2^-49 of one
+// common largest value: a row 2^34 times the others left those with 15 bits, one 2^50 times with none.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -32,10 +36,17 @@ typedef short i16x8 __attribute__((ext_vector_type(8)));
 #define MCCLX_GLOBAL __attribute__((address_space(1)))
 #define MCCLX_LDS __attribute__((address_space(3)))
 
-// Element types of a product's operands: bf16, f16, or fp32 as two planes of f16.
-struct Bf16 { typedef __bf16 T; typedef bf16x4 T4; typedef bf16x8 T8; static constexpr int kPlanes = 1; };
-struct F16 { typedef _Float16 T; typedef f16x4 T4; typedef f16x8 T8; static constexpr int kPlanes = 1; };
-struct Split { typedef _Float16 T; typedef f16x4 T4; typedef f16x8 T8; static constexpr int kPlanes = 2; };
+// Element types of a product's operands: bf16, f16, or fp32 as three planes of bf16.  kDzScale: what dz, which lies in -1 .. 1, is multiplied
+// by before it is rounded to them.  f16 has most of its numbers below 2^14, and its rare tokens' p keep 11 bits down to 2^-28; fp32's planes
+// get the size of the matrices.
+struct Bf16 { typedef __bf16 T; typedef bf16x4 T4; typedef bf16x8 T8; static constexpr int kPlanes = 1; static constexpr float kDzScale = 0x1p14f; };
+struct F16 { typedef _Float16 T; typedef f16x4 T4; typedef f16x8 T8; static constexpr int kPlanes = 1; static constexpr float kDzScale = 0x1p14f; };
+struct Split { typedef __bf16 T; typedef bf16x4 T4; typedef bf16x8 T8; static constexpr int kPlanes = 3; static constexpr float kDzScale = 0x1p50f; };
+constexpr int kMostPlanes = 3;
+// Of pass n of a split product, the planes of p and q, small terms first.
+constexpr int kPasses = 6;
+__device__ __forceinline__ uint32_t plane_of_p(uint32_t pass) { return 0x121 >> 2 * pass & 3; }   // 1 0 2 0 1 0
+__device__ __forceinline__ uint32_t plane_of_q(uint32_t pass) { return 0x049 >> 2 * pass & 3; }   // 1 2 0 1 0 0
 
 // c += a b on the matrix cores, c in accumulation registers.  Named here, because the compiler, left to choose, moves a
 // tile's accumulators to and fro between the two register files in every step; volatile, so that a step's products,
@@ -43,7 +54,7 @@ struct Split { typedef _Float16 T; typedef f16x4 T4; typedef f16x8 T8; static co
 // instructions: `settle`, and a and b come from LDS reads, never from an instruction right in front of them.
 template <class E>
 __device__ __forceinline__ void mfma(const i16x8& a, const i16x8& b, f32x4& c) {
-    if constexpr (std::is_same_v<E, Bf16>)
+    if constexpr (std::is_same_v<typename E::T, __bf16>)
         asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     else
         asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
@@ -192,9 +203,9 @@ struct Reader {
 };
 
 struct Operand {
-    const void* plane[2];  // the second one of a split operand
-    uint64_t ld;           // elements
-    uint32_t rows, cols;   // in memory
+    const void* plane[kMostPlanes];
+    uint64_t ld;          // elements
+    uint32_t rows, cols;  // in memory
 };
 struct GemmArgs {
     Operand p, q;
@@ -206,7 +217,7 @@ struct GemmArgs {
     float *max_sum, *target_logit;  // [tiles_p][tokens][2], [tokens]
     const int64_t* target;
     const float *lse, *row_scale, *scales;  // scales: see Scale
-    void* out[2];
+    void* out[kMostPlanes];
     uint64_t out_ld;
     uint32_t first;         // vocabulary entry of p = 0 (logits)
     uint32_t vocab, tokens;
@@ -214,7 +225,6 @@ struct GemmArgs {
 };
 // Device floats behind `scales`.
 enum Scale { kInverseHidden = 0, kInverseWeight = 1, kGradient = 2, kScales = 4 };
-constexpr float kDzScale = 16384.f;  // dz lies in -1 .. 1, and f16 has most of its numbers below that: its rare tokens' p keep 11 bits down to 2^-28
 
 enum Epilogue { kLse, kDz, kStore, kPartial };
 
@@ -280,7 +290,8 @@ __global__ void __launch_bounds__(256, TILE == kTile || STAGES > kStages ? 1 : 2
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, wave_p = wave % 2, wave_q = wave / 2;
     const uint32_t all = (a.k + kStep - 1) / kStep, share = ((all + a.splits - 1) / a.splits + STAGES - 1) / STAGES * STAGES;
     const uint32_t begin = split * share < all ? split * share : all, count = all - begin < share ? all - begin : share;
-    constexpr int kPasses = E::kPlanes == 2 ? 3 : 1;  // lo hi, hi lo, hi hi
+    constexpr bool kSplit = E::kPlanes > 1;
+    constexpr uint32_t kTurns = kSplit ? kPasses : 1;
     constexpr int kPair = 2 * TILE / 32;              // loads of two stages, where both operands lie alike
 
     Loader<P_OUTER, TILE> load_p;
@@ -296,14 +307,15 @@ __global__ void __launch_bounds__(256, TILE == kTile || STAGES > kStages ? 1 : 2
     const uint32_t rounds = (count + STAGES - 1) / STAGES;
     uint32_t load_step = 0, load_pass = 0;  // the next step to load
     auto start = [&] {
-        load_p.start(a.p.plane[E::kPlanes == 2 && load_pass == 0], begin, a.p.ld, p0, a.p.rows);
-        load_q.start(a.q.plane[E::kPlanes == 2 && load_pass == 1], begin, a.q.ld, q0, a.q.rows);
+        auto plane = [](const Operand& o, uint32_t n) { return !kSplit || n == 0 ? o.plane[0] : n == 1 ? o.plane[1] : o.plane[2]; };
+        load_p.start(plane(a.p, plane_of_p(load_pass)), begin, a.p.ld, p0, a.p.rows);
+        load_q.start(plane(a.q, plane_of_q(load_pass)), begin, a.q.ld, q0, a.q.rows);
     };
     auto advance = [&](int stage) {  // past the loads of a stage
         ++load_step;
         if (P_OUTER || stage % 2) load_p.advance(load_step < count);
         if (Q_OUTER || stage % 2) load_q.advance(load_step < count);
-        if (kPasses > 1 && load_step == rounds * STAGES && load_pass + 1 < kPasses) {
+        if (kSplit && load_step == rounds * STAGES && load_pass + 1 < kTurns) {
             load_step = 0;
             ++load_pass;
             start();
@@ -379,20 +391,8 @@ __global__ void __launch_bounds__(256, TILE == kTile || STAGES > kStages ? 1 : 2
             });
             advance(stage);
         };
-        for (int pass = 0; pass < kPasses; ++pass) {
-            for (uint32_t t = 0; t < rounds; ++t) {
-                each<STAGES>(step);
-            }
-            settle();
-            if constexpr (E::kPlanes == 2) {
-                const float unit = pass == 1 ? 0x1p-11f : 1.f;
-#pragma unroll
-                for (int i = 0; i < kFrags; ++i)
-#pragma unroll
-                    for (int j = 0; j < kFrags; ++j) acc[i][j] *= unit;
-                settle();
-            }
-        }
+        for (uint32_t t = 0; t < rounds * kTurns; ++t) each<STAGES>(step);
+        settle();
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // LDS is free
 
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(256, TILE == kTile || STAGES > kStages ? 1 : 2
     const uint32_t p_lane = p0 + wave_p * kWaveTile + lane / 16 * 4, q_lane = q0 + wave_q * kWaveTile + lane % 16;
     const uint32_t p_pair = p0 + wave_p * kWaveTile + lane / 32 * 16 + lane / 16 % 2 * 8;  // of eight_of's values
     if constexpr (EPI == kLse || EPI == kDz) {
-        if constexpr (E::kPlanes == 2) {
+        if constexpr (kSplit) {
             // (the product of both inverses may overflow where a logit does not)
             const float unit_h = a.scales[kInverseHidden], unit_w = a.scales[kInverseWeight], unit = unit_h * unit_w;
             const bool one = unit > 1e-36f && unit < 1e36f;
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(256, TILE == kTile || STAGES > kStages ? 1 : 2
         for (int j = 0; j < kFrags; ++j) {
             const uint32_t q = q_lane + 16 * j;
             const bool in = q < a.tokens;
-            const float lse = in ? a.lse[q] : 0.f, scale = in ? a.row_scale[q] * kDzScale : 0.f, minus = -lse * kLog2e;
+            const float lse = in ? a.lse[q] : 0.f, scale = in ? a.row_scale[q] * E::kDzScale : 0.f, minus = -lse * kLog2e;
 #pragma unroll
             for (int i = 0; i < kFrags; ++i)
 #pragma unroll
@@ -500,31 +500,34 @@ __global__ void __launch_bounds__(256, TILE == kTile || STAGES > kStages ? 1 : 2
 #pragma unroll
             for (int i = 0; i < kFrags; i += 2) {
                 const uint64_t at = (uint64_t)q * a.out_ld + p_pair + 16 * i;
-                typename E::T4 hi[2];
+                f32x4 rest[2] = {acc[i][j], acc[i + 1][j]};
 #pragma unroll
-                for (int k = 0; k < 2; ++k) hi[k] = __builtin_convertvector(acc[i + k][j], typename E::T4);
-                *reinterpret_cast<i32x4*>(static_cast<typename E::T*>(a.out[0]) + at) = eight_of(hi[0], hi[1]);
-                if constexpr (E::kPlanes == 2) {
-                    f16x4 lo[2];
+                for (int plane = 0; plane < E::kPlanes; ++plane) {
+                    typename E::T4 part[2];
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) lo[k] = __builtin_convertvector((acc[i + k][j] - __builtin_convertvector(hi[k], f32x4)) * 2048.f, f16x4);
-                    *reinterpret_cast<i32x4*>(static_cast<_Float16*>(a.out[1]) + at) = eight_of(lo[0], lo[1]);
+                    for (int k = 0; k < 2; ++k) {
+                        part[k] = __builtin_convertvector(rest[k], typename E::T4);
+                        rest[k] -= __builtin_convertvector(part[k], f32x4);
+                    }
+                    *reinterpret_cast<i32x4*>(static_cast<typename E::T*>(a.out[plane]) + at) = eight_of(part[0], part[1]);
                 }
             }
         }
     } else if constexpr (EPI == kStore) {
-        const float gradient = a.scales[kGradient], unit = E::kPlanes == 2 ? a.scales[kInverseHidden] : 1.f;
+        const float gradient = a.scales[kGradient], unit = kSplit ? a.scales[kInverseHidden] : 1.f;
+        // (dz's power of two first, then the matrix's: the sum in the numbers it stands for, which fp32 holds)
+        auto result = [&](const f32x4& v) { return v * (1.f / E::kDzScale) * unit * gradient; };
 #pragma unroll
         for (int j = 0; j < kFrags; ++j) {
             const uint32_t q = q_lane + 16 * j;
             const bool in = q < a.rows_out;
-            if constexpr (E::kPlanes == 2) {
+            if constexpr (kSplit) {
                 typedef f32x4 Loose __attribute__((aligned(4)));
                 float* row = static_cast<float*>(a.out[0]) + (uint64_t)q * a.out_ld;
 #pragma unroll
                 for (int i = 0; i < kFrags; ++i) {
                     const uint32_t p = p_lane + 16 * i;
-                    const f32x4 v = acc[i][j] * gradient * unit;
+                    const f32x4 v = result(acc[i][j]);
                     if (in && p + 4 <= a.out_ld) {
                         *reinterpret_cast<Loose*>(row + p) = v;
                     } else if (in) {
@@ -540,8 +543,8 @@ __global__ void __launch_bounds__(256, TILE == kTile || STAGES > kStages ? 1 : 2
 #pragma unroll
                 for (int i = 0; i < kFrags; i += 2) {
                     const uint32_t p = p_pair + 16 * i;
-                    const i32x4 v = eight_of(__builtin_convertvector(acc[i][j] * gradient, typename E::T4),
-                                             __builtin_convertvector(acc[i + 1][j] * gradient, typename E::T4));
+                    const i32x4 v = eight_of(__builtin_convertvector(result(acc[i][j]), typename E::T4),
+                                             __builtin_convertvector(result(acc[i + 1][j]), typename E::T4));
                     if (in && p + 8 <= a.out_ld) {
                         *reinterpret_cast<Loose*>(row + p) = v;
                     } else if (in) {
@@ -689,7 +692,7 @@ __global__ void __launch_bounds__(1024) row_scale_kernel(const float* grad, int 
         count = block_sum(count, scratch);
         factor = reduction == MCCLX_LOSS_SUM ? *grad : count == 0.f ? 0.f : *grad / count;
     }
-    if (threadIdx.x == 0) scales[kGradient] = factor / kDzScale;
+    if (threadIdx.x == 0) scales[kGradient] = factor;
 }
 
 // The lanes of a block over a matrix: 2^shift to a row, for rows of `packets` packets.
@@ -709,7 +712,7 @@ struct Copies {
     const void* from[2];
     uint64_t ld[2];
     uint32_t rows[2];
-    void *to[2], *second[2];  // fp32: the planes
+    void* to[2];              // (fp32: the planes, one behind the other)
     uint32_t inverse[2];      // fp32: which of `scales`
     uint32_t cols, wide;
     uint32_t* bits;           // fp32: kLargest floats' a matrix
@@ -776,17 +779,18 @@ __global__ void __launch_bounds__(256) largest_kernel(Copies a) {
     top = largest_of_block(top);
     if (threadIdx.x == 0) a.bits[blockIdx.y * kLargest + blockIdx.x] = top;
 }
-// The two f16 planes of an fp32 matrix, and the inverse of its scale.
+// The three bf16 planes of an fp32 matrix, and the inverse of its scale.
 __global__ void __launch_bounds__(256) split_kernel(Copies a) {
     const float* const from = static_cast<const float*>(a.from[blockIdx.y]);
-    _Float16 *const hi = static_cast<_Float16*>(a.to[blockIdx.y]), *const lo = static_cast<_Float16*>(a.second[blockIdx.y]);
+    __bf16* const to = static_cast<__bf16*>(a.to[blockIdx.y]);
     const uint64_t ld = a.ld[blockIdx.y];
     const uint32_t rows = a.rows[blockIdx.y], cols = a.cols, wide = a.wide;
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < kLargest; i += 256) most = larger(most, a.bits[blockIdx.y * kLargest + i + threadIdx.x]);
-    // 2^e with the largest value below 2^15 after it; 0 and the smallest numbers get the largest e
-    int e = 14 - ((int)(largest_of_block(most) >> 23) - 127);
+    // 2^e with the largest value below 2^51 after it (a sum of 2^24 products of two such values stays below 2^126); 0 and the smallest
+    // numbers get the largest e
+    int e = 50 - ((int)(largest_of_block(most) >> 23) - 127);
     e = e > 126 ? 126 : e;
     const float s = __builtin_ldexpf(1.f, e);
     if (blockIdx.x == 0 && threadIdx.x == 0) a.scales[a.inverse[blockIdx.y]] = __builtin_ldexpf(1.f, -e);
@@ -805,20 +809,22 @@ __global__ void __launch_bounds__(256) split_kernel(Copies a) {
                     if (c * 8 + r < cols) v[r] = p[r];
             }
             v *= s;
-            const f16x8 h = __builtin_convertvector(v, f16x8);
-            f32x8 rest = (v - __builtin_convertvector(h, f32x8)) * 2048.f;
 #pragma unroll
-            for (int r = 0; r < 8; ++r) rest[r] = __builtin_isfinite(v[r]) ? rest[r] : 0.f;  // (an infinity or a NaN is all in its upper half)
-            *reinterpret_cast<f16x8*>(hi + row * wide + c * 8) = h;
-            *reinterpret_cast<f16x8*>(lo + row * wide + c * 8) = __builtin_convertvector(rest, f16x8);
+            for (int plane = 0; plane < Split::kPlanes; ++plane) {
+                const bf16x8 part = __builtin_convertvector(v, bf16x8);
+                *reinterpret_cast<bf16x8*>(to + ((uint64_t)plane * rows + row) * wide + c * 8) = part;
+                const f32x8 rest = v - __builtin_convertvector(part, f32x8);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) v[r] = __builtin_isfinite(v[r]) ? rest[r] : 0.f;  // (an infinity or a NaN is all in its first plane)
+            }
         }
 }
 
 // dh from its partial sums, four columns a lane, eight loads under way at a time.
-template <class T, bool SPLIT>
+template <class E, class T>
 __global__ void __launch_bounds__(256) join_hidden_kernel(const float* sums, uint32_t splits, uint64_t split_stride, uint32_t wide, uint32_t tokens,
                                                           uint32_t width, const float* scales, T* out) {
-    const float gradient = scales[kGradient], unit = SPLIT ? scales[kInverseWeight] : 1.f;
+    const float gradient = scales[kGradient], unit = E::kPlanes > 1 ? scales[kInverseWeight] : 1.f;
     const Spread at((width + 3) / 4);
     for (uint64_t row = at.row; row < tokens; row += at.rows)
         for (uint32_t c = at.lane * 4; c < width; c += 4u << at.shift) {
@@ -833,7 +839,7 @@ __global__ void __launch_bounds__(256) join_hidden_kernel(const float* sums, uin
                 for (int k = 0; k < 8; ++k) v += part[k];
             }
             for (; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(from + s * split_stride);
-            v = v * gradient * unit;
+            v = v * (1.f / E::kDzScale) * unit * gradient;
             T* to = out + row * width + c;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -853,7 +859,7 @@ struct Plan {
     uint32_t wide;                    // columns of a packed operand
     uint32_t tiles_tokens, tiles_vocab;  // of 256
     uint32_t tile, cus;                  // of the logits' products; of the device
-    uint64_t h, w;                    // packed operands (both planes), bytes from the start
+    uint64_t h, w;                    // packed operands (all planes), bytes from the start
     uint64_t scales, bits, row_scale, target_logit, losses, max_sum, dz, sums;
     uint32_t piece, splits, sum_wide; // vocabulary entries of a piece
     uint64_t bytes;
@@ -897,7 +903,7 @@ Plan plan_for(const LossArgs& a, bool backward, int cus) {
         at += up(bytes, 256);
         return was;
     };
-    const uint64_t planes = l.split ? 2 : 1;
+    const uint64_t planes = l.split ? Split::kPlanes : 1;
     l.scales = take(kScales * 4);
     if (l.split) l.bits = take(2 * kLargest * 4);
     if (l.pack_h) l.h = take(planes * a.tokens * l.wide * 2);
@@ -908,9 +914,8 @@ Plan plan_for(const LossArgs& a, bool backward, int cus) {
         l.max_sum = take((uint64_t)lse_parts(l, a.vocab) * a.tokens * 8);
     } else {
         l.row_scale = take((uint64_t)a.tokens * 4);
-        // dz of a piece: 512 MB, and at least 16 tiles.  (Backward of 4096 tokens, 50257 x 768 f32: 2.97 ms at 256 MB, which the last
-        // cache holds, 2.79 at 512, 2.74 at 1024; of 8192, 131072 x 4096 bf16: 19.4, 19.4, 19.2.  At 64 MB 4096 tokens, 32000 x 768 f32,
-        // take 1.6 times as long.)
+        // dz of a piece: 512 MB, and at least 16 tiles.  (Backward of 4096 tokens, 50257 x 768 f32: 5.67 ms at 256 MB, which the last
+        // cache holds, 4.91 at 512, 4.84 at 1024; of 8192, 131072 x 4096 bf16: 19.4, 19.4, 19.2.)
         const uint64_t rows = up(a.tokens, l.tile);
         uint64_t tiles = (512ull << 20) / (rows * kTile * 2 * planes);
         tiles = tiles < 16 ? 16 : tiles;
@@ -953,8 +958,8 @@ void clear(Run& r, void* p, uint64_t bytes) {
 // The operands as the products read them.
 template <class E>
 void operands(Run& r, const LossArgs& a, const Plan& l, char* work, Operand* h, Operand* w) {
-    *h = {{a.hidden, nullptr}, a.hidden_ld, a.tokens, a.width};
-    *w = {{a.weight, nullptr}, a.weight_ld, a.vocab, a.width};
+    *h = {{a.hidden}, a.hidden_ld, a.tokens, a.width};
+    *w = {{a.weight}, a.weight_ld, a.vocab, a.width};
     Copies c = {};
     c.cols = a.width;
     c.wide = l.wide;
@@ -966,15 +971,15 @@ void operands(Run& r, const LossArgs& a, const Plan& l, char* work, Operand* h, 
         c.ld[n] = o->ld;
         c.rows[n] = o->rows;
         c.to[n] = work + at;
-        c.second[n] = E::kPlanes == 2 ? work + at + (uint64_t)o->rows * l.wide * 2 : nullptr;
         c.inverse[n] = inverse;
-        *o = {{c.to[n], c.second[n]}, l.wide, o->rows, l.wide};
+        for (int i = 0; i < E::kPlanes; ++i) o->plane[i] = work + at + (uint64_t)i * o->rows * l.wide * 2;
+        o->ld = o->cols = l.wide;
         ++n;
     };
     if (l.pack_h) copy(l.h, kInverseHidden, h);
     if (l.pack_w) copy(l.w, kInverseWeight, w);
     if (n == 0) return;
-    if constexpr (E::kPlanes == 2) {
+    if constexpr (E::kPlanes > 1) {
         largest_kernel<<<dim3(kLargest, n), dim3(256), 0, r.st>>>(c);
         r.done();
         split_kernel<<<dim3(2048, n), dim3(256), 0, r.st>>>(c);
@@ -1031,7 +1036,7 @@ void forward(Run& r, const LossArgs& a, const Plan& l) {
     g.tokens = a.tokens;
     logits<E, kLse>(r, g, l, large_logits(l, l.tiles_vocab), a.vocab, a.tokens);
     // (more tokens a block where that makes one of it and saves a launch, unless it would have too much to read: forward of 64 tokens,
-    // 2000 x 256 f32, 24.3 us, in two launches 26.5; 32000 x 1024 bf16, 250 parts, 22.1, 22.6; 131072 x 1024, 1024 parts, stays at two)
+    // 32000 x 1024 bf16, 250 parts, 22.1, 22.6; 131072 x 1024, 1024 parts, stays at two)
     const uint32_t parts = lse_parts(l, a.vocab), each = a.tokens > 16 && a.tokens <= 64 && parts <= 512 ? 64 : 16;
     const JoinArgs join = {g.max_sum, g.target_logit, a.target, a.ignore_index, parts, a.tokens, a.vocab, a.reduction == MCCLX_LOSS_MEAN, a.lse,
                            a.reduction == MCCLX_LOSS_NONE ? a.loss : reinterpret_cast<float*>(work + l.losses), a.loss, each,
@@ -1047,7 +1052,7 @@ void forward(Run& r, const LossArgs& a, const Plan& l) {
 template <class E>
 void backward(Run& r, const LossArgs& a, const Plan& l) {
     typedef typename E::T T;
-    typedef std::conditional_t<E::kPlanes == 2, float, T> Out;
+    typedef std::conditional_t<(E::kPlanes > 1), float, T> Out;
     char* work = static_cast<char*>(a.workspace);
     Operand h, w;
     operands<E>(r, a, l, work, &h, &w);
@@ -1056,7 +1061,8 @@ void backward(Run& r, const LossArgs& a, const Plan& l) {
     row_scale_kernel<<<dim3(1), dim3(1024), 0, r.st>>>(a.grad, a.reduction, a.target, a.ignore_index, a.tokens, a.vocab, row_scale, scales);
     r.done();
     const uint64_t rows = up(a.tokens, l.tile);
-    const Operand dz = {{work + l.dz, work + l.dz + rows * l.piece * 2}, l.piece, (uint32_t)rows, l.piece};
+    Operand dz = {{}, l.piece, (uint32_t)rows, l.piece};
+    for (int i = 0; i < E::kPlanes; ++i) dz.plane[i] = work + l.dz + i * rows * l.piece * 2;
     for (uint32_t first = 0; first < a.vocab; first += l.piece) {
         const uint32_t some = a.vocab - first < l.piece ? a.vocab - first : l.piece;
         Operand wp = w;
@@ -1071,8 +1077,7 @@ void backward(Run& r, const LossArgs& a, const Plan& l) {
         g.lse = a.lse_in;
         g.row_scale = row_scale;
         g.scales = scales;
-        g.out[0] = work + l.dz;
-        g.out[1] = const_cast<void*>(dz.plane[1]);
+        for (int i = 0; i < E::kPlanes; ++i) g.out[i] = const_cast<void*>(dz.plane[i]);
         g.out_ld = l.piece;
         g.first = first;
         g.vocab = a.vocab;
@@ -1124,7 +1129,7 @@ void backward(Run& r, const LossArgs& a, const Plan& l) {
         }
     }
     if (a.dhidden) {
-        join_hidden_kernel<Out, E::kPlanes == 2><<<dim3(a.tokens < 4096 ? a.tokens : 4096), dim3(256), 0, r.st>>>(
+        join_hidden_kernel<E, Out><<<dim3(a.tokens < 4096 ? a.tokens : 4096), dim3(256), 0, r.st>>>(
             reinterpret_cast<const float*>(work + l.sums), l.splits, (uint64_t)l.tiles_tokens * kTile * l.sum_wide, l.sum_wide, a.tokens, a.width, scales,
             static_cast<Out*>(a.dhidden));
         r.done();

@@ -284,7 +284,8 @@ def linear_cross_entropy_forward(hidden, weight, target, ignore_index: int = -10
     logarithm of each token's sum of exponentials.  hidden is (..., width), weight (vocabulary, width),
     target (...) int64.  Targets equal to ignore_index have the loss 0 and do not count in the mean, which is NaN
     where none is left; a target outside the vocabulary makes its loss, and what its gradient reaches, NaN.  Both
-    results are float32."""
+    results are float32.  float32 matrices are multiplied with float32's precision, for values down to 2^-100 of the
+    largest finite one of their matrix."""
     q = _q(queue)
     _on_gpu(q, hidden, "hidden")
     lse = hidden.new_empty(hidden.shape[:-1], dtype=torch.float32)
