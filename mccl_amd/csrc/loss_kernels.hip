@@ -661,7 +661,8 @@ __global__ void __launch_bounds__(1024) reduce_loss_kernel(JoinArgs a) {
 }
 
 // What each row's dz is multiplied by, in -1 .. 1 (NaN where its target does not exist, as its loss is), and the factor
-// that the gradients then lack (one block).
+// that the gradients then lack (one block).  With a gradient a token, the factor is the largest finite one's size, and a row whose own is
+// no number, or infinite, takes that as it is: it reaches that row of dhidden, and dweight, to which every row adds.
 __global__ void __launch_bounds__(1024) row_scale_kernel(const float* grad, int reduction, const int64_t* target, int64_t ignore, uint32_t tokens,
                                                          uint32_t vocab, float* row_scale, float* scales) {
     __shared__ float scratch[16];
@@ -670,18 +671,18 @@ __global__ void __launch_bounds__(1024) row_scale_kernel(const float* grad, int 
     if (reduction == MCCLX_LOSS_NONE) {
         float top = 0.f;
         for (uint32_t i = threadIdx.x; i < tokens; i += 1024) {
-            const float g = target[i] == ignore ? 0.f : __builtin_fabsf(grad[i]);
-            top = !(g <= top) ? g : top;  // (a NaN comes through)
+            const float g = __builtin_fabsf(grad[i]);
+            top = target[i] != ignore && __builtin_isfinite(g) ? __builtin_fmaxf(top, g) : top;
         }
-        for (int x = 32; x; x >>= 1) {
-            const float o = __shfl_xor(top, x);
-            top = !(o <= top) ? o : top;
-        }
+        for (int x = 32; x; x >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
         if (threadIdx.x % 64 == 0) scratch[threadIdx.x / 64] = top;
         __syncthreads();
-        for (int i = 0; i < 16; ++i) top = !(scratch[i] <= top) ? scratch[i] : top;
-        factor = top;
-        for (uint32_t i = threadIdx.x; i < tokens; i += 1024) row_scale[i] = target[i] == ignore || top == 0.f ? 0.f : grad[i] / top * there(i);
+        for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, scratch[i]);
+        factor = top == 0.f ? 1.f : top;
+        for (uint32_t i = threadIdx.x; i < tokens; i += 1024) {
+            const float g = grad[i];
+            row_scale[i] = target[i] == ignore ? 0.f : (__builtin_isfinite(g) ? g / factor : g) * there(i);
+        }
     } else {
         float count = 0.f;
         for (uint32_t i = threadIdx.x; i < tokens; i += 1024) {

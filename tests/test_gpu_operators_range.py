@@ -1,5 +1,5 @@
-"""linear_cross_entropy of float32 matrices whose rows, columns, probabilities and gradients lie many powers of two apart: what
-is large in one row must not cost another its precision.
+"""linear_cross_entropy of float32 matrices whose rows, columns, probabilities and gradients lie many powers of two apart, and
+gradients that are no numbers: what is large, or lost, in one row must not cost another its precision.
 
 Bounds.  As in test_gpu_operators_loss.py, first order, but weighted by the probabilities: an entry of the vocabulary that nobody
 expects does not add to a logarithm's error, however large its logit.  A float32 product is off by its own rounding and by at most as
@@ -13,7 +13,7 @@ from test_gpu_operators_loss import make
 
 pytestmark = pytest.mark.gpu
 
-F32 = torch.float32
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 U = O.U32
 NOTHING = 2.0 ** -120
 
@@ -97,3 +97,28 @@ def test_float32_gradients_of_entries_that_nobody_expects(ops, e):
 def test_float32_gradients_of_tokens_far_apart(ops):
     h, w, t = make(60, 300, 64, F32, seed=23)
     check(ops, h, w, t, gradients(60) * torch.logspace(-30, 3, 60, device="cuda"))
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=str)
+def test_a_gradient_that_is_no_number_stays_in_its_row(ops, dtype, value):
+    h, w, t = make(300, 520, 64, dtype, seed=24)
+    t[5], t[9] = 3, -100
+    grad = gradients(300)
+    grad[5] = 0.0
+    lse = ops.linear_cross_entropy_forward(h, w, t)[1]
+    clean, _ = ops.linear_cross_entropy_backward(grad, h, w, t, lse, reduction="none")
+    for row in (5, 9):
+        bad = grad.clone()
+        bad[row] = value
+        dh, dw = ops.linear_cross_entropy_backward(bad, h, w, t, lse, reduction="none")
+        rest = torch.arange(300) != row
+        assert torch.equal(dh[rest], clean[rest])
+        if row == 5:
+            assert not torch.isfinite(dh[5]).any() and not torch.isfinite(dw).any()
+        else:                   # an ignored token's gradient reaches nobody
+            assert not dh[9].any() and torch.isfinite(dw).all()
+    only = torch.zeros(300, device="cuda")
+    only[5] = value
+    dh, _ = ops.linear_cross_entropy_backward(only, h, w, t, lse, reduction="none")
+    assert not torch.isfinite(dh[5]).any() and not dh[torch.arange(300) != 5].any()
