@@ -140,10 +140,12 @@ def _norm_forward(q, x, residual, weight, bias, p, seed, offset, eps, keep_sum):
     return y, s, mean, rstd
 
 
-def _norm_backward(q, dy, ds, s, mean, rstd, weight, p, seed, offset, seam, with_bias):
+def _norm_backward(q, dy, ds, s, mean, rstd, weight, p, seed, offset, seam, bias_dtype):
+    """bias_dtype: dbias's, None: no dbias."""
     native = _reader()
     if native is not None:
-        done = native._norm_backward(q.handle.value, q.device, dy, ds, s, mean, rstd, weight, p, seed, offset, seam, with_bias)
+        done = native._norm_backward(q.handle.value, q.device, dy, ds, s, mean, rstd, weight, p, seed, offset, seam,
+                                     -1 if bias_dtype is None else _DTYPE.get(bias_dtype, -2))
         if done is not None:
             L.check(done[0])
             return done[1:]
@@ -155,13 +157,17 @@ def _norm_backward(q, dy, ds, s, mean, rstd, weight, p, seed, offset, seam, with
         _same(s, ds, "ds")
         ds, _, _, ds_stride = _rows(q, ds, "ds")
     param = _params(q, s, cols, (weight, "weight"))
+    if bias_dtype is not None:
+        if bias_dtype not in ((s.dtype, torch.float32) if weight is None else (weight.dtype,)):
+            raise MCCLError(f"[MCCL] bias: dtype {bias_dtype} beside {s.dtype if weight is None else weight.dtype}", L.ERR_UNSUPPORTED)
+        param = _DTYPE[bias_dtype]
     _stats(q, mean, rows, "mean")
     _stats(q, rstd, rows, "rstd")
     lib = L.lib()
     dx = _like(s)
     dresidual = torch.empty_like(dx) if seam else None
     dweight = torch.empty_like(weight) if weight is not None else None
-    dbias = None if not with_bias else torch.empty_like(weight) if weight is not None else s.new_empty(cols)
+    dbias = None if bias_dtype is None else s.new_empty(cols, dtype=bias_dtype)
     nbytes = lib.mcclx_layer_norm_workspace_bytes(q.handle, rows, cols)
     work = s.new_empty(nbytes, dtype=torch.uint8)
     a = L.Norm(dtype_code(s), param, rows, cols, 0.0, p, seed, offset, _ptr(weight), None, mean.data_ptr(), rstd.data_ptr(),
@@ -178,10 +184,15 @@ def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5, queue=None)
     return y, mean, rstd
 
 
-def layer_norm_backward(dy, x, mean, rstd, weight=None, with_bias: bool = True, queue=None):
-    """(dx, dweight, dbias); dweight is None without a weight, dbias where with_bias is false.
-    Sums over the rows are taken in the same order in every call."""
-    dx, _, dweight, dbias = _norm_backward(_q(queue), dy, None, x, mean, rstd, weight, 0.0, 0, 0, False, with_bias)
+def _bias_dtype(with_bias: bool, bias_dtype, weight, x):
+    return None if not with_bias else bias_dtype if bias_dtype is not None else x.dtype if weight is None else weight.dtype
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, with_bias: bool = True, queue=None, *, bias_dtype=None):
+    """(dx, dweight, dbias); dweight is None without a weight, dbias where with_bias is false.  bias_dtype is the
+    bias's where there is no weight to tell it (None: x's).  Sums over the rows are taken in the same order in every call."""
+    dx, _, dweight, dbias = _norm_backward(_q(queue), dy, None, x, mean, rstd, weight, 0.0, 0, 0, False,
+                                           _bias_dtype(with_bias, bias_dtype, weight, x))
     return dx, dweight, dbias
 
 
@@ -194,10 +205,11 @@ def dropout_add_layer_norm_forward(x, residual, weight=None, bias=None, p: float
 
 
 def dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, weight=None, p: float = 0.0, seed: int = 0, offset: int = 0,
-                                    with_bias: bool = True, queue=None):
-    """(dx, dresidual, dweight, dbias) from the gradients of y and of s (ds may be None)."""
+                                    with_bias: bool = True, queue=None, *, bias_dtype=None):
+    """(dx, dresidual, dweight, dbias) from the gradients of y and of s (ds may be None); the rest as in
+    layer_norm_backward."""
     p, seed, offset = _mask(p, seed, offset)
-    return _norm_backward(_q(queue), dy, ds, s, mean, rstd, weight, p, seed, offset, True, with_bias)
+    return _norm_backward(_q(queue), dy, ds, s, mean, rstd, weight, p, seed, offset, True, _bias_dtype(with_bias, bias_dtype, weight, s))
 
 
 # ---- dropout ----------------------------------------------------------------------
@@ -329,14 +341,15 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, queue):
         y, mean, rstd = layer_norm_forward(x, weight, bias, eps, queue)
         ctx.save_for_backward(x, mean, rstd, weight)
-        ctx.with_bias, ctx.queue = bias is not None, queue
+        ctx.bias_dtype, ctx.queue = None if bias is None else bias.dtype, queue
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, mean, rstd, weight = ctx.saved_tensors
-        return (*layer_norm_backward(dy, x, mean, rstd, weight, ctx.with_bias, ctx.queue), None, None)
+        return (*layer_norm_backward(dy, x, mean, rstd, weight, ctx.bias_dtype is not None, ctx.queue, bias_dtype=ctx.bias_dtype),
+                None, None)
 
 
 class _Dropout(torch.autograd.Function):
@@ -357,7 +370,7 @@ class _Seam(torch.autograd.Function):
     def forward(ctx, x, residual, weight, bias, p, seed, offset, eps, queue):
         y, s, mean, rstd = dropout_add_layer_norm_forward(x, residual, weight, bias, p, seed, offset, eps, queue)
         ctx.save_for_backward(s, mean, rstd, weight)
-        ctx.mask, ctx.with_bias, ctx.queue = (p, seed, offset), bias is not None, queue
+        ctx.mask, ctx.bias_dtype, ctx.queue = (p, seed, offset), None if bias is None else bias.dtype, queue
         ctx.set_materialize_grads(False)
         return y, s
 
@@ -367,7 +380,8 @@ class _Seam(torch.autograd.Function):
         s, mean, rstd, weight = ctx.saved_tensors
         if dy is None:
             dy = torch.zeros_like(s)
-        return (*dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, weight, *ctx.mask, with_bias=ctx.with_bias, queue=ctx.queue),
+        return (*dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, weight, *ctx.mask, ctx.bias_dtype is not None, ctx.queue,
+                                                 bias_dtype=ctx.bias_dtype),
                 None, None, None, None, None)
 
 

@@ -291,6 +291,29 @@ def test_other_streams_and_recordings(ops):
             assert torch.equal(a, c)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+def test_a_float32_bias_without_a_weight_has_a_float32_gradient(ops, dtype):
+    """Its sum over the rows is not rounded to the rows' type on the way."""
+    x, dy, b = make((300, 200), dtype, 100), make((300, 200), dtype, 101), make((200,), F32, 102)
+    _, mean, rstd = ops.layer_norm_forward(x, None, b)
+    want, bound = O.f64(dy).sum(0), 330 * O.U32 * np.abs(O.f64(dy)).sum(0)
+    for mine, theirs in ((x, dy), (x[:, 1:], dy[:, 1:])):      # (adjacent rows, and rows that lie apart)
+        last = slice(200 - mine.shape[1], 200)
+        leaf = b[last].clone().requires_grad_()
+        ops.layer_norm(mine, None, leaf).backward(theirs)
+        O.close(leaf.grad, want[last], bound[last], "layer_norm")
+        leaf = b[last].clone().requires_grad_()
+        ops.dropout_add_layer_norm(mine, mine, None, leaf)[0].backward(theirs)
+        O.close(leaf.grad, want[last], bound[last], "seam")
+    db = ops.layer_norm_backward(dy, x, mean, rstd, bias_dtype=F32)[2]
+    O.close(db, want, bound, "dbias")
+    assert ops.layer_norm_backward(dy, x, mean, rstd)[2].dtype == dtype
+    from mccl_amd import MCCLError
+    for weight, bad in ((None, torch.float64), (None, F16 if dtype == BF16 else BF16), (x[0], F32), (b, dtype)):
+        with pytest.raises(MCCLError, match=r"^\[MCCL\] bias"):
+            ops.layer_norm_backward(dy, x, mean, rstd, weight, bias_dtype=bad)
+
+
 def test_launches_are_counted(ops):
     from mccl_amd import kernels
     q = kernels.hip_kernels_init(0)
