@@ -140,11 +140,11 @@ def _norm_forward(q, x, residual, weight, bias, p, seed, offset, eps, keep_sum):
     return y, s, mean, rstd
 
 
-def _norm_backward(q, dy, ds, s, mean, rstd, weight, p, seed, offset, seam, bias_dtype):
+def _norm_backward(q, dy, ds, s, mean, rstd, weight, p, seed, offset, with_residual, bias_dtype):
     """bias_dtype: dbias's, None: no dbias."""
     native = _reader()
     if native is not None:
-        done = native._norm_backward(q.handle.value, q.device, dy, ds, s, mean, rstd, weight, p, seed, offset, seam,
+        done = native._norm_backward(q.handle.value, q.device, dy, ds, s, mean, rstd, weight, p, seed, offset, with_residual,
                                      -1 if bias_dtype is None else _DTYPE.get(bias_dtype, -2))
         if done is not None:
             L.check(done[0])
@@ -165,7 +165,7 @@ def _norm_backward(q, dy, ds, s, mean, rstd, weight, p, seed, offset, seam, bias
     _stats(q, rstd, rows, "rstd")
     lib = L.lib()
     dx = _like(s)
-    dresidual = torch.empty_like(dx) if seam else None
+    dresidual = torch.empty_like(dx) if with_residual else None
     dweight = torch.empty_like(weight) if weight is not None else None
     dbias = None if bias_dtype is None else s.new_empty(cols, dtype=bias_dtype)
     nbytes = lib.mcclx_layer_norm_workspace_bytes(q.handle, rows, cols)
@@ -205,11 +205,12 @@ def dropout_add_layer_norm_forward(x, residual, weight=None, bias=None, p: float
 
 
 def dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, weight=None, p: float = 0.0, seed: int = 0, offset: int = 0,
-                                    with_bias: bool = True, queue=None, *, bias_dtype=None):
-    """(dx, dresidual, dweight, dbias) from the gradients of y and of s (ds may be None); the rest as in
-    layer_norm_backward."""
+                                    with_bias: bool = True, queue=None, *, bias_dtype=None, with_residual: bool = True):
+    """(dx, dresidual, dweight, dbias) from the gradients of y and of s (ds may be None); dresidual is None where
+    with_residual is false, the rest as in layer_norm_backward."""
     p, seed, offset = _mask(p, seed, offset)
-    return _norm_backward(_q(queue), dy, ds, s, mean, rstd, weight, p, seed, offset, True, _bias_dtype(with_bias, bias_dtype, weight, s))
+    return _norm_backward(_q(queue), dy, ds, s, mean, rstd, weight, p, seed, offset, with_residual,
+                          _bias_dtype(with_bias, bias_dtype, weight, s))
 
 
 # ---- dropout ----------------------------------------------------------------------
@@ -381,7 +382,7 @@ class _Seam(torch.autograd.Function):
         if dy is None:
             dy = torch.zeros_like(s)
         return (*dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, weight, *ctx.mask, ctx.bias_dtype is not None, ctx.queue,
-                                                 bias_dtype=ctx.bias_dtype),
+                                                 bias_dtype=ctx.bias_dtype, with_residual=ctx.needs_input_grad[1]),
                 None, None, None, None, None)
 
 
@@ -422,7 +423,8 @@ def dropout(x, p: float, masks: Optional[MaskStream] = None, residual=None, queu
 
 def dropout_add_layer_norm(x, residual, weight=None, bias=None, p: float = 0.0, masks: Optional[MaskStream] = None,
                            eps: float = 1e-5, queue=None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Differentiable (y, s): s = residual + dropout(x) with the next mask of `masks`, y = layer_norm(s)."""
+    """Differentiable (y, s): s = residual + dropout(x) with the next mask of `masks` (residual None: without the sum),
+    y = layer_norm(s)."""
     return _Seam.apply(x, residual, weight, bias, p, *_next(p, masks, "dropout_add_layer_norm"), eps, queue)
 
 

@@ -314,6 +314,19 @@ def test_a_float32_bias_without_a_weight_has_a_float32_gradient(ops, dtype):
             ops.layer_norm_backward(dy, x, mean, rstd, weight, bias_dtype=bad)
 
 
+def test_a_seam_without_a_residual(ops):
+    x, w, b, dy = (make(s, F32, 125 + i) for i, s in enumerate([(20, 96), (96,), (96,), (20, 96)]))
+    zero = torch.zeros_like(x)
+    got = []
+    for res in (None, zero):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        y, s = ops.dropout_add_layer_norm(leaves[0], res, leaves[1], leaves[2], 0.2, ops.MaskStream(4))
+        torch.autograd.backward([y, s], [dy, dy])
+        got.append([y, s] + [t.grad for t in leaves])
+    for a, c in zip(*got):
+        assert torch.equal(a, c)
+
+
 def test_launches_are_counted(ops):
     from mccl_amd import kernels
     q = kernels.hip_kernels_init(0)
