@@ -80,7 +80,8 @@ py::object norm_forward(uintptr_t handle, int device, const at::Tensor& x, const
 }
 
 py::object norm_backward(uintptr_t handle, int device, const at::Tensor& dy, const Maybe& ds, const at::Tensor& s, const at::Tensor& mean,
-                         const at::Tensor& rstd, const Maybe& weight, double p, uint64_t seed, uint64_t offset, bool with_residual, int bias_dtype) {
+                         const at::Tensor& rstd, const Maybe& weight, double p, uint64_t seed, uint64_t offset, bool with_x, bool with_residual,
+                         bool with_weight, int bias_dtype) {
     if (!matrix(s, device) || !like(dy, s, device) || (ds && !like(*ds, s, device)) || !parameter(weight, s, device)) return py::none();
     mcclx_norm a = arguments(s, weight, std::nullopt, p, seed, offset);
     if (bias_dtype != -1) {  // (-1: no gradient of a bias)
@@ -89,10 +90,10 @@ py::object norm_backward(uintptr_t handle, int device, const at::Tensor& dy, con
     }
     if (!statistic(mean, static_cast<int64_t>(a.rows), device) || !statistic(rstd, static_cast<int64_t>(a.rows), device)) return py::none();
     const at::AutoDispatchBelowAutograd guard;
-    const at::Tensor dx = fresh_like(s);
-    Maybe dresidual, dweight, dbias;
+    Maybe dx, dresidual, dweight, dbias;
+    if (with_x) dx = fresh_like(s);
     if (with_residual) dresidual = fresh_like(s);
-    if (weight) dweight = fresh_like(*weight);
+    if (weight && with_weight) dweight = fresh_like(*weight);
     if (bias_dtype != -1) dbias = at::empty({s.size(-1)}, a.param_dtype == a.dtype ? s.options() : s.options().dtype(at::kFloat));
     a.workspace_bytes = mcclx_layer_norm_workspace_bytes(context(handle), a.rows, a.cols);
     const at::Tensor work = dev::empty_bytes(static_cast<int64_t>(a.workspace_bytes), device);
@@ -102,7 +103,7 @@ py::object norm_backward(uintptr_t handle, int device, const at::Tensor& dy, con
     a.s = s.data_ptr();
     a.dy = dy.data_ptr();
     a.ds = address(ds);
-    a.dx = dx.data_ptr();
+    a.dx = address(dx);
     a.dresidual = address(dresidual);
     a.dweight = address(dweight);
     a.dbias = address(dbias);

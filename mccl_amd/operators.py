@@ -140,12 +140,12 @@ def _norm_forward(q, x, residual, weight, bias, p, seed, offset, eps, keep_sum):
     return y, s, mean, rstd
 
 
-def _norm_backward(q, dy, ds, s, mean, rstd, weight, p, seed, offset, with_residual, bias_dtype):
+def _norm_backward(q, dy, ds, s, mean, rstd, weight, p, seed, offset, with_x, with_residual, with_weight, bias_dtype):
     """bias_dtype: dbias's, None: no dbias."""
     native = _reader()
     if native is not None:
-        done = native._norm_backward(q.handle.value, q.device, dy, ds, s, mean, rstd, weight, p, seed, offset, with_residual,
-                                     -1 if bias_dtype is None else _DTYPE.get(bias_dtype, -2))
+        done = native._norm_backward(q.handle.value, q.device, dy, ds, s, mean, rstd, weight, p, seed, offset, with_x, with_residual,
+                                     with_weight, -1 if bias_dtype is None else _DTYPE.get(bias_dtype, -2))
         if done is not None:
             L.check(done[0])
             return done[1:]
@@ -164,14 +164,14 @@ def _norm_backward(q, dy, ds, s, mean, rstd, weight, p, seed, offset, with_resid
     _stats(q, mean, rows, "mean")
     _stats(q, rstd, rows, "rstd")
     lib = L.lib()
-    dx = _like(s)
-    dresidual = torch.empty_like(dx) if with_residual else None
-    dweight = torch.empty_like(weight) if weight is not None else None
+    dx = _like(s) if with_x else None
+    dresidual = _like(s) if with_residual else None
+    dweight = torch.empty_like(weight) if with_weight and weight is not None else None
     dbias = None if bias_dtype is None else s.new_empty(cols, dtype=bias_dtype)
     nbytes = lib.mcclx_layer_norm_workspace_bytes(q.handle, rows, cols)
     work = s.new_empty(nbytes, dtype=torch.uint8)
     a = L.Norm(dtype_code(s), param, rows, cols, 0.0, p, seed, offset, _ptr(weight), None, mean.data_ptr(), rstd.data_ptr(),
-               None, None, None, sr.data_ptr(), dyr.data_ptr(), _ptr(ds), dx.data_ptr(), _ptr(dresidual), _ptr(dweight),
+               None, None, None, sr.data_ptr(), dyr.data_ptr(), _ptr(ds), _ptr(dx), _ptr(dresidual), _ptr(dweight),
                _ptr(dbias), 0, 0, s_stride, dy_stride, ds_stride, work.data_ptr(), nbytes)
     L.check(lib.mcclx_layer_norm_backward(q.handle, _stream(q), C.byref(a)))
     return dx, dresidual, dweight, dbias
@@ -188,10 +188,12 @@ def _bias_dtype(with_bias: bool, bias_dtype, weight, x):
     return None if not with_bias else bias_dtype if bias_dtype is not None else x.dtype if weight is None else weight.dtype
 
 
-def layer_norm_backward(dy, x, mean, rstd, weight=None, with_bias: bool = True, queue=None, *, bias_dtype=None):
-    """(dx, dweight, dbias); dweight is None without a weight, dbias where with_bias is false.  bias_dtype is the
-    bias's where there is no weight to tell it (None: x's).  Sums over the rows are taken in the same order in every call."""
-    dx, _, dweight, dbias = _norm_backward(_q(queue), dy, None, x, mean, rstd, weight, 0.0, 0, 0, False,
+def layer_norm_backward(dy, x, mean, rstd, weight=None, with_bias: bool = True, queue=None, *, bias_dtype=None,
+                        with_x: bool = True, with_weight: bool = True):
+    """(dx, dweight, dbias), None where not wanted; dweight is None without a weight too.  bias_dtype is the bias's where
+    there is no weight to tell it (None: x's).  Sums over the rows are taken in the same order in every call; without dweight and
+    dbias the pass is one launch."""
+    dx, _, dweight, dbias = _norm_backward(_q(queue), dy, None, x, mean, rstd, weight, 0.0, 0, 0, with_x, False, with_weight,
                                            _bias_dtype(with_bias, bias_dtype, weight, x))
     return dx, dweight, dbias
 
@@ -205,11 +207,11 @@ def dropout_add_layer_norm_forward(x, residual, weight=None, bias=None, p: float
 
 
 def dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, weight=None, p: float = 0.0, seed: int = 0, offset: int = 0,
-                                    with_bias: bool = True, queue=None, *, bias_dtype=None, with_residual: bool = True):
-    """(dx, dresidual, dweight, dbias) from the gradients of y and of s (ds may be None); dresidual is None where
-    with_residual is false, the rest as in layer_norm_backward."""
+                                    with_bias: bool = True, queue=None, *, bias_dtype=None, with_x: bool = True,
+                                    with_residual: bool = True, with_weight: bool = True):
+    """(dx, dresidual, dweight, dbias) from the gradients of y and of s (ds may be None), as in layer_norm_backward."""
     p, seed, offset = _mask(p, seed, offset)
-    return _norm_backward(_q(queue), dy, ds, s, mean, rstd, weight, p, seed, offset, with_residual,
+    return _norm_backward(_q(queue), dy, ds, s, mean, rstd, weight, p, seed, offset, with_x, with_residual, with_weight,
                           _bias_dtype(with_bias, bias_dtype, weight, s))
 
 
@@ -342,15 +344,16 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, queue):
         y, mean, rstd = layer_norm_forward(x, weight, bias, eps, queue)
         ctx.save_for_backward(x, mean, rstd, weight)
-        ctx.bias_dtype, ctx.queue = None if bias is None else bias.dtype, queue
+        ctx.bias_dtype, ctx.queue = bias.dtype if ctx.needs_input_grad[2] else None, queue
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, mean, rstd, weight = ctx.saved_tensors
-        return (*layer_norm_backward(dy, x, mean, rstd, weight, ctx.bias_dtype is not None, ctx.queue, bias_dtype=ctx.bias_dtype),
-                None, None)
+        need = ctx.needs_input_grad
+        return (*layer_norm_backward(dy, x, mean, rstd, weight, need[2], ctx.queue, bias_dtype=ctx.bias_dtype, with_x=need[0],
+                                     with_weight=need[1]), None, None)
 
 
 class _Dropout(torch.autograd.Function):
@@ -371,7 +374,7 @@ class _Seam(torch.autograd.Function):
     def forward(ctx, x, residual, weight, bias, p, seed, offset, eps, queue):
         y, s, mean, rstd = dropout_add_layer_norm_forward(x, residual, weight, bias, p, seed, offset, eps, queue)
         ctx.save_for_backward(s, mean, rstd, weight)
-        ctx.mask, ctx.bias_dtype, ctx.queue = (p, seed, offset), None if bias is None else bias.dtype, queue
+        ctx.mask, ctx.bias_dtype, ctx.queue = (p, seed, offset), bias.dtype if ctx.needs_input_grad[3] else None, queue
         ctx.set_materialize_grads(False)
         return y, s
 
@@ -381,8 +384,9 @@ class _Seam(torch.autograd.Function):
         s, mean, rstd, weight = ctx.saved_tensors
         if dy is None:
             dy = torch.zeros_like(s)
-        return (*dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, weight, *ctx.mask, ctx.bias_dtype is not None, ctx.queue,
-                                                 bias_dtype=ctx.bias_dtype, with_residual=ctx.needs_input_grad[1]),
+        need = ctx.needs_input_grad
+        return (*dropout_add_layer_norm_backward(dy, ds, s, mean, rstd, weight, *ctx.mask, need[3], ctx.queue, bias_dtype=ctx.bias_dtype,
+                                                 with_x=need[0], with_residual=need[1], with_weight=need[2]),
                 None, None, None, None, None)
 
 

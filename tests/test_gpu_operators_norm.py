@@ -314,6 +314,32 @@ def test_a_float32_bias_without_a_weight_has_a_float32_gradient(ops, dtype):
             ops.layer_norm_backward(dy, x, mean, rstd, weight, bias_dtype=bad)
 
 
+def test_what_is_frozen_costs_nothing(ops):
+    """A backward pass writes what somebody asks for: without the parameters' gradients it is one launch."""
+    from mccl_amd import kernels
+    q = kernels.hip_kernels_init(0)
+    x, res, w, b, dy = (make(s, BF16, 120 + i) for i, s in enumerate([(300, 200), (300, 200), (200,), (200,), (300, 200)]))
+
+    def gradients(call, *wanted):
+        leaves = [t.clone().requires_grad_(want) for t, want in zip((x, res, w, b), wanted)]
+        y = call(*leaves)
+        n = q.launch_count()
+        y.backward(dy)
+        return [t.grad for t in leaves], q.launch_count() - n
+
+    norm = lambda x, res, w, b: ops.layer_norm(x, w, b)
+    seam = lambda x, res, w, b: ops.dropout_add_layer_norm(x, res, w, b, 0.3, ops.MaskStream(5))[0]
+    for call in (norm, seam):
+        every, launches = gradients(call, True, call is seam, True, True)
+        assert launches == 2
+        for wanted in ((True, False, False, False), (False, False, True, False), (False, False, False, True), (True, False, False, True)) + (
+                ((False, True, False, False), (True, True, False, False)) if call is seam else ()):
+            got, launches = gradients(call, *wanted)
+            assert launches == (2 if wanted[2] or wanted[3] else 1), wanted
+            for a, e, want in zip(got, every, wanted):
+                assert torch.equal(a, e) if want else a is None
+
+
 def test_a_seam_without_a_residual(ops):
     x, w, b, dy = (make(s, F32, 125 + i) for i, s in enumerate([(20, 96), (96,), (96,), (20, 96)]))
     zero = torch.zeros_like(x)
