@@ -248,12 +248,14 @@ def dropout_backward(dy, p: float, seed: int, offset: int = 0, queue=None):
 class MaskStream:
     """Hands out a (seed, offset) for each use of dropout.  Ranks of one training run share the seed and
     differ in rank, which sits in the offset's upper bits; state_dict() is what a checkpoint keeps, and
-    a run that continues from it draws the masks it would have drawn."""
+    a run that continues from it draws the masks it would have drawn.  A stream that was given a rank keeps it whatever
+    state it loads: all ranks may resume from one rank's checkpoint.  Without one (None: rank 0) it takes the state's."""
 
-    def __init__(self, seed: int, rank: int = 0):
-        if not 0 <= rank < 1 << 16:
+    def __init__(self, seed: int, rank: Optional[int] = None):
+        if rank is not None and not 0 <= rank < 1 << 16:
             raise MCCLError(f"[MCCL] MaskStream: rank {rank} outside 0..65535")
-        self.seed, self.rank, self.count = int(seed) & _M64, rank, 0
+        self.seed, self.rank, self.count = int(seed) & _M64, rank or 0, 0
+        self._own_rank = rank is not None
 
     def next(self) -> Tuple[int, int]:
         offset = (self.rank << 48) | (self.count & ((1 << 48) - 1))
@@ -264,7 +266,9 @@ class MaskStream:
         return {"seed": self.seed, "rank": self.rank, "count": self.count}
 
     def load_state_dict(self, state: dict) -> None:
-        self.seed, self.rank, self.count = state["seed"], state["rank"], state["count"]
+        self.seed, self.count = state["seed"], state["count"]
+        if not self._own_rank:
+            self.rank = state["rank"]
 
 
 # ---- the loss ------------------------------------------------------------------------

@@ -49,3 +49,22 @@ def test_no_fallback_without_a_queue(monkeypatch):
     monkeypatch.setattr(kernels, "_default", None)
     with pytest.raises(MCCLError, match="not called"):
         operators.layer_norm_forward(torch.ones(2, 2))
+
+
+def test_ranks_that_resume_from_one_state_keep_masks_of_their_own():
+    """The usual checkpoint: rank 0 saves, every rank loads."""
+    from mccl_amd import operators
+    saved = operators.MaskStream(7, rank=0)
+    saved.next()
+    state = saved.state_dict()
+    following = saved.next()
+    drawn = []
+    for rank in range(4):
+        stream = operators.MaskStream(99, rank=rank)
+        stream.load_state_dict(state)
+        assert (stream.seed, stream.rank, stream.count) == (7, rank, 1)
+        drawn.append(stream.next())
+    assert drawn[0] == following and len(set(drawn)) == 4
+    alone = operators.MaskStream(0)                   # one that names no rank takes the state's
+    alone.load_state_dict(operators.MaskStream(7, rank=3).state_dict())
+    assert alone.next() == operators.MaskStream(7, rank=3).next()
