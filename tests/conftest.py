@@ -3,8 +3,9 @@ import sys
 
 import pytest
 
-# libmcclx checks every launch's pointers against their allocations when this is set
-os.environ.setdefault("MCCLX_VALIDATE", "1")
+# libmcclx checks every launch's pointers against their allocations when this is set.  Set whatever the environment says: tests of
+# refusals pass sizes that run past their tensors, and such a call must end at that check.
+os.environ["MCCLX_VALIDATE"] = "1"
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 

@@ -68,3 +68,14 @@ def test_ranks_that_resume_from_one_state_keep_masks_of_their_own():
     alone = operators.MaskStream(0)                   # one that names no rank takes the state's
     alone.load_state_dict(operators.MaskStream(7, rank=3).state_dict())
     assert alone.next() == operators.MaskStream(7, rank=3).next()
+
+
+def test_the_tests_check_every_pointer_whatever_the_environment_says():
+    """Some refusals that they ask for are told by a range check alone."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    out = subprocess.run([sys.executable, "-c", "import conftest, os; print(os.environ['MCCLX_VALIDATE'])"], cwd=here, text=True, capture_output=True,
+                         env={**os.environ, "MCCLX_VALIDATE": "0"}, check=True).stdout
+    assert out.strip() == "1"
