@@ -531,12 +531,13 @@ __global__ void __launch_bounds__(256) norm_backward_long_kernel(NormBackwardArg
     }
 }
 
-// dweight and dbias from their partial sums: a block to 32 columns, its 32 half waves take the parts in turn, eight
+// dweight and dbias from their partial sums, columns `first` on: a block to 32 columns, its 32 half waves take the parts in turn, eight
 // loads under way at a time (512 parts of 4096 columns 4.8 us).
 template <class P>
-__global__ void __launch_bounds__(1024) norm_join_kernel(const float* partial, uint32_t parts, uint32_t cols, P* dweight, P* dbias) {
+__global__ void __launch_bounds__(1024) norm_join_kernel(const float* partial, uint32_t parts, uint32_t cols, uint32_t first, P* dweight, P* dbias) {
     __shared__ float both[32][33];
-    const uint32_t c = blockIdx.x * 32 + threadIdx.x % 32, slice = threadIdx.x / 32;
+    first += blockIdx.x * 32;
+    const uint32_t c = first + threadIdx.x % 32, slice = threadIdx.x / 32;
     P* out = blockIdx.y ? dbias : dweight;
     if (!out) return;
     const float* from = partial + (uint64_t)blockIdx.y * cols + (c < cols ? c : cols - 1);
@@ -552,7 +553,7 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(const float* partial, u
     __syncthreads();
     float v[1] = {both[threadIdx.x % 32][slice]};  // column `slice` of the block, a slice a lane
     row_sum<32>(v, nullptr);
-    if (threadIdx.x % 32 == 0 && blockIdx.x * 32 + slice < cols) out[blockIdx.x * 32 + slice] = (P)v[0];
+    if (threadIdx.x % 32 == 0 && first + slice < cols) out[first + slice] = (P)v[0];
 }
 
 // A packet a lane.  4096 x 768 f32 with a residual 7.5 us, 5.0 TB/s, 16384 x 8192 bf16 94 us, 5.7 TB/s: the generator's twenty products a packet
@@ -571,7 +572,8 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs a, uint32_t pa
 
 // ---- launches ------------------------------------------------------------------------
 
-constexpr uint64_t kRowsALaunch = 1u << 21;            // a grid holds 2^32 lanes at most
+constexpr uint64_t kRowsALaunch = 1u << 21;            // a grid holds 2^32 lanes at most, and silently leaves out the others
+constexpr uint32_t kJoinedALaunch = 1u << 26;          // columns; 32 lanes each, of one dimension
 constexpr uint32_t kForwardMost = 1024 * 2 * kPacket;  // columns that a block of norm_forward_kernel holds
 
 template <class T, class P, int LANES, int NV>
@@ -656,11 +658,12 @@ int backward_for(hipStream_t st, NormBackwardArgs a) {
             norm_backward_long_kernel<T, P, false><<<grid, dim3(256), 0, st>>>(a, sums);
         launches = 2;
     }
-    if (a.dweight || a.dbias) {
-        norm_join_kernel<P><<<dim3((a.cols + 31) / 32, 2), dim3(1024), 0, st>>>(a.partial, a.parts, a.cols, static_cast<P*>(a.dweight),
-                                                                               static_cast<P*>(a.dbias));
-        ++launches;
-    }
+    if (a.dweight || a.dbias)
+        for (uint32_t first = 0; first < a.cols; first += kJoinedALaunch, ++launches) {
+            const uint32_t some = a.cols - first < kJoinedALaunch ? a.cols - first : kJoinedALaunch;
+            norm_join_kernel<P><<<dim3((some + 31) / 32, 2), dim3(1024), 0, st>>>(a.partial, a.parts, a.cols, first, static_cast<P*>(a.dweight),
+                                                                                 static_cast<P*>(a.dbias));
+        }
     return launches;
 }
 

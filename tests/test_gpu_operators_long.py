@@ -100,6 +100,18 @@ def test_more_rows_than_a_launch_takes(ops):
     O.close(db, O.f64(dy.double().sum(0)), (rows + 30) * O.U32 * O.f64(dy.double().abs().sum(0)), "dbias")
 
 
+def test_sums_of_more_columns_than_one_launch_takes(ops):
+    """A grid holds 2^32 lanes, and the parameters' sums take 32 a column."""
+    cols = (1 << 27) + 40
+    x, dy = filled(1, cols), filled(1, cols, seed=2)
+    w = torch.ones(cols, dtype=BF16, device="cuda")
+    mean, rstd = torch.full((1,), 0.25, device="cuda"), torch.full((1,), 1.5, device="cuda")
+    _, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, w)
+    assert torch.equal(db, dy[0])                     # one row: its sum is itself
+    u = (x[0].float() - 0.25) * 1.5
+    assert torch.equal(dw, (dy[0].float() * u).bfloat16())
+
+
 # what is short in one call goes in small tiles, what is long in large ones
 @pytest.mark.parametrize("tokens", [5, 300])
 @pytest.mark.parametrize("dtype,vocab,width", [(BF16, 530001, 4096), (F32, 270001, 4096)], ids=str)
