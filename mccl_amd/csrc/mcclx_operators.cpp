@@ -46,6 +46,9 @@ struct Checker {
                       (unsigned long long)*stride);
         else if (!rc && *stride > (1ull << 40))
             rc = fail(MCCLX_ERR_INVALID, "%s: rows lie %llu elements apart", what, (unsigned long long)*stride);
+        // (2^56 elements are past every address; and the next product, in bytes, cannot wrap)
+        else if (!rc && n > 1 && n - 1 > (1ull << 56) / (*stride ? *stride : 1))
+            rc = fail(MCCLX_ERR_INVALID, "%s: %llu rows that lie %llu elements apart", what, (unsigned long long)n, (unsigned long long)*stride);
         if (!rc && n && mcclx_ctx_validates(ctx)) rc = mcclx_check_range(p, ((n - 1) * *stride + cols) * size, what);
     }
     void flat(const char* what, const void* p, bool wanted, uint64_t size, uint64_t n) {

@@ -410,3 +410,17 @@ def test_refusals(ops):
     assert lib.mcclx_layer_norm_backward(q.handle, None, C.byref(a)) == L.ERR_INVALID and "workspace" in L.last_error()
     assert lib.mcclx_layer_norm_forward(q.handle, None, None) == L.ERR_INVALID
     torch.cuda.synchronize()
+
+
+def test_rows_further_apart_than_addresses_reach(ops):
+    """(rows - 1) * stride in bytes is a multiple of 2^64: no range check sees anything of it."""
+    from mccl_amd import _lib as L, kernels
+    q, lib = kernels.hip_kernels_init(0), L.lib()
+    rows = (1 << 24) + 1
+    x, s = torch.ones(1, 8, device="cuda"), torch.ones(rows, device="cuda")
+    work = torch.empty(int(lib.mcclx_layer_norm_workspace_bytes(q.handle, rows, 8)), dtype=torch.uint8, device="cuda")
+    a = L.Norm(L.F32, L.F32, rows, 8)
+    a.s, a.dy, a.mean, a.rstd = x.data_ptr(), x.data_ptr(), s.data_ptr(), s.data_ptr()
+    a.s_stride = a.dy_stride = 1 << 40
+    a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
+    assert lib.mcclx_layer_norm_backward(q.handle, None, C.byref(a)) == L.ERR_INVALID and "elements apart" in L.last_error()
