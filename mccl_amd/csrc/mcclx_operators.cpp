@@ -231,11 +231,12 @@ int mcclx_layer_norm_backward(mcclx_ctx* ctx, void* stream, const mcclx_norm* a)
     k.parts = mcclx::norm_backward_parts(a->rows, (uint32_t)a->cols, cus);
     const uint64_t need = some ? mcclx::norm_backward_scratch(a->rows, (uint32_t)a->cols, cus) : 0;
     if (need) {
-        c.flat("workspace", a->workspace, true, 16, 1);
-        if (c.rc) return c.rc;
         if (a->workspace_bytes < need)
             return fail(MCCLX_ERR_INVALID, "workspace of %llu bytes, %llu are needed", (unsigned long long)a->workspace_bytes,
                         (unsigned long long)need);
+        c.flat("workspace", a->workspace, true, 16, 1);  // (its alignment)
+        c.flat("workspace", a->workspace, true, 1, need);
+        if (c.rc) return c.rc;
     }
     k.dy = a->dy;
     k.ds = a->ds;

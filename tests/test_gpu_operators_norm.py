@@ -424,3 +424,17 @@ def test_rows_further_apart_than_addresses_reach(ops):
     a.s_stride = a.dy_stride = 1 << 40
     a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
     assert lib.mcclx_layer_norm_backward(q.handle, None, C.byref(a)) == L.ERR_INVALID and "elements apart" in L.last_error()
+
+
+def test_a_workspace_that_ends_early(ops):
+    """16 MB are needed and claimed, 512 bytes are there (in an allocation of at most 2 MB, torch's unit for small tensors)."""
+    from mccl_amd import _lib as L, kernels
+    q, lib = kernels.hip_kernels_init(0), L.lib()
+    x, s = torch.ones(4096, 8192, dtype=BF16, device="cuda"), torch.ones(4096, device="cuda")
+    w, small = torch.ones(8192, dtype=BF16, device="cuda"), torch.empty(512, dtype=torch.uint8, device="cuda")
+    need = lib.mcclx_layer_norm_workspace_bytes(q.handle, 4096, 8192)
+    assert need > 2 << 20
+    a = L.Norm(L.BF16, L.BF16, 4096, 8192)
+    a.s, a.dy, a.mean, a.rstd, a.weight, a.dweight = x.data_ptr(), x.data_ptr(), s.data_ptr(), s.data_ptr(), w.data_ptr(), w.data_ptr()
+    a.workspace, a.workspace_bytes = small.data_ptr(), need
+    assert lib.mcclx_layer_norm_backward(q.handle, None, C.byref(a)) == L.ERR_INVALID and "workspace" in L.last_error()
