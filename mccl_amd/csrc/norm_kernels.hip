@@ -244,8 +244,11 @@ __global__ void __launch_bounds__(LANES <= 64 ? 256 : LANES) norm_forward_kernel
 #pragma unroll
     for (int j = 0; j < NV; ++j) t[j] = to_f32<T>(at.template get<T>(x, j));
     // The parameters are on their way while the row is summed (8 x 1024 bf16 3.0 us, behind the sums 3.3; 16384 x 4096 bf16 41.4, 43.0), unless
-    // that takes registers which waves need (2048 x 16384 f32 62.7, 48.9; 65536 x 512 f32 with the seam 102, 100).
-    constexpr bool kEarly = LANES < 1024 && (sizeof(T) == 2 || !SEAM);
+    // that takes registers which waves need: blocks of 1024 (2048 x 16384 f32 62.7, 48.9), f32 rows with the seam (65536 x 512 102, 100),
+    // three packets a lane (32768 x 1280 bf16 33.9, 30.5, with f32 parameters 40.5, 30.0; 8192 x 1280 f32 20.6, 17.0; 146 registers, and 47), and f32
+    // parameters beside long 16-bit rows, with the seam those of more than a wave (16384 x 6144 98, 90.5, seam 163, 154; 65536 x 2048 seam 204,
+    // 196; but 16384 x 2560 28.4, 29.3, 16384 x 1024 seam 22.4, 22.9).
+    constexpr bool kEarly = LANES < 1024 && NV < 3 && (sizeof(T) == sizeof(P) ? sizeof(T) == 2 || !SEAM : LANES <= (SEAM ? 64 : 256));
     Raw<P> w[NV], b[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
