@@ -459,7 +459,9 @@ MCCLX_API int mcclx_allgather_replay(mcclx_ctx* ctx, int world, void* const* out
  * context's device (NULL: the default one) and not on the reduce queue: a model's
  * kernels need no order with a gradient bucket that is under way.  A bucket that
  * waits for the stream (mcclx_queue_wait_stream) waits for them as for any producer.
- * They launch kernels only, allocate nothing and may be recorded into a graph.
+ * They launch kernels only, allocate nothing and may be recorded into a graph, which
+ * keeps their arguments: a dropout's seed and offset too, so that every replay draws
+ * the mask of the recording.
  * Sums and statistics are held in fp32, every output is rounded once.  Matrices are
  * rows of `cols` adjacent elements; an input's rows lie `*_stride` elements apart
  * (0: `cols`), an output's are adjacent.  Element alignment is enough, 16 bytes

@@ -9,7 +9,8 @@ masks of dropout.  Every arithmetic launch is a hand-written HIP kernel inside l
 The kernels run on torch's current stream, not on the reduce queue: they are the producers
 whose gradients a bucket's allreduce waits for.  A queue (`hip_kernels_init`) must exist: it
 names the device and counts the launches.  Scratch memory comes from torch's allocator for
-each call.  A call may be recorded into a graph.
+each call.  A call may be recorded into a graph, which keeps its arguments: the seed and offset of a dropout too, so that
+every replay draws the mask of the recording.  A training step that is replayed keeps its dropouts outside the graph, or p at 0.
 
 Tensors are matrices of rows: the last dimension is the row.  Rows may lie further apart than
 they are long (a slice of a wider tensor is read in place); any other layout is copied first.
