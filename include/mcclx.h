@@ -523,8 +523,10 @@ MCCLX_API int mcclx_dropout(mcclx_ctx* ctx, void* stream, int dtype, uint64_t ro
  * reaches NaN.  `grad` is the gradient of the loss: one float, or one a token for
  * MCCLX_LOSS_NONE.  fp32 matrices, and dz in between the products of a backward
  * pass, are multiplied with fp32's precision, whatever the sizes of other rows, for
- * values down to 2^-100 of the largest finite one of their matrix (dz: of 1).  For
- * 16-bit matrices dz is rounded to their type, f16 after a factor of 2^14. */
+ * values down to 2^-100 of the largest finite one of their matrix (dz: of 1 times the
+ * largest finite gradient); an infinity in an fp32 matrix makes NaN of the logits that it
+ * reaches.  For 16-bit matrices dz is rounded to their type, f16 after a factor of 2^14
+ * over that gradient. */
 enum { MCCLX_LOSS_NONE = 0, MCCLX_LOSS_MEAN = 1, MCCLX_LOSS_SUM = 2 };
 typedef struct {
     int32_t dtype;     /* of hidden, weight and their gradients */

@@ -618,6 +618,7 @@ void forward_for(hipStream_t st, const NormForwardArgs& a) {
 // a row of partial sums (4096 x 768 f32 in blocks of four rows / eight 12.3 / 11.2 us, 1000 x 4096 f16 in one / two 18.8 / 15.7,
 // with the seam 4099 x 1111 f16 in one / five 24.1 / 24.9, 16384 x 4096 bf16 in one / two 141 / 131; one number that was lost is 16384 x 4096 bf16
 // without the seam, 85.0 / 86.8).  The narrowest rows stay at eight waves, for calls of few rows (1000 x 64 6.0 us, at sixteen 7.1).
+// Blocks of 960 and 1024 lanes have 128 registers a lane: f32 rows with the seam spill 8 to 24 bytes there (128, 192, 256 and 512 lanes).
 struct Shape {
     uint32_t lanes, packets, rows;
 };
