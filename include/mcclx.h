@@ -521,7 +521,8 @@ MCCLX_API int mcclx_dropout(mcclx_ctx* ctx, void* stream, int dtype, uint64_t ro
  * `ignore_index`, whose loss is 0; the mean is over those that are not (NaN where
  * none is left).  A target outside 0 .. vocab - 1 makes its loss and what its gradient
  * reaches NaN.  `grad` is the gradient of the loss: one float, or one a token for
- * MCCLX_LOSS_NONE.  fp32 matrices, and dz in between the products of a backward
+ * MCCLX_LOSS_NONE.  (An ignored token's hidden row is multiplied by zeros for dweight, and
+ * has to be finite for that.)  fp32 matrices, and dz in between the products of a backward
  * pass, are multiplied with fp32's precision, whatever the sizes of other rows, for
  * values down to 2^-100 of the largest finite one of their matrix (dz: of 1 times the
  * largest finite gradient); an infinity in an fp32 matrix makes NaN of the logits that it

@@ -84,6 +84,24 @@ def test_float32_matrices_of_rows_far_apart(ops, where, e, shape):
     check(ops, h, w, t, gradients(len(h)))
 
 
+def test_float32_matrices_with_a_large_row_each(ops):
+    """Padding 2^100 times as large as the tokens, and an entry 2^100 times as large as the others: both matrices at the end of their range."""
+    h, w, t = make(60, 300, 64, F32, seed=25)
+    h[7] *= 2.0 ** 100
+    w[11] *= 2.0 ** 100
+    t[7] = -100
+    grad = gradients(60)
+    loss, lse = ops.linear_cross_entropy_forward(h, w, t, reduction="none")
+    dh, dw = ops.linear_cross_entropy_backward(grad, h, w, t, lse, reduction="none")
+    rest = torch.arange(60) != 7
+    wl, wlse, wh, ww, el, elw, eh, ew = oracle(h[rest], w, t[rest], O.f64(grad)[rest.numpy()])
+    O.close(lse[rest], wlse, elw, "lse")
+    O.close(loss[rest], wl, el, "loss")
+    O.close(dh[rest], wh, eh, "dhidden")
+    O.close(dw, ww, ew, "dweight")
+    assert float(loss[7]) == 0.0 and not dh[7].any()
+
+
 @pytest.mark.parametrize("e", [30, 60])
 def test_float32_gradients_of_entries_that_nobody_expects(ops, e):
     """Half of the vocabulary has probabilities around 2^-e; those rows of dweight are held to their own size."""
