@@ -60,7 +60,7 @@ __device__ __forceinline__ void mfma(const i16x8& a, const i16x8& b, f32x4& c) {
         asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 // Loads 16 bytes a lane from a buffer straight into LDS at `to` + OFFSET (the same in all lanes) + 16 lane; what lies past
-// the buffer's end reads as zero.  In assembly, because the compiler would wait for all such loads at the next transposing
+// the buffer's end, lane_offset and the scalar offset together, reads as zero.  In assembly, because the compiler would wait for all such loads at the next transposing
 // read; they return nothing in registers, and `arrive` does the waiting.  (m0 and its use need an instruction between them.)
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 template <int OFFSET>
